@@ -181,7 +181,8 @@ int vl_knn_tile_parts(const uint16_t* rows_bf16, int64_t n, int dim_pad, const f
  * int8 [n, code_ld] with code_ld = dim rounded up to a multiple of 16 and zeros behind dim, one fp32 scale s and the
  * sum of c^2 (int32).  s = max|x| / 127 rounded to fp32; c = the whole number nearest to the exact x / s, ties to even
  * (0 where s is 0).  A row with an infinity or a NaN has the scale NaN and the codes 0.  dim <= 131072, codes 16-byte
- * aligned.  Rows come and go as VL_TYPE_F32, _BF16 or _F16, their row strides (ld, out_ld) count elements.
+ * aligned.  Rows come and go as VL_TYPE_F32, _BF16 or _F16, their row strides (ld, out_ld) count elements.  Every pointer
+ * is aligned to its elements, and rows of a result do not overlap: other calls are refused.
  *
  * vl_quant_write: row r of rows [m, dim] goes to place ids[r], or first_row + r when ids == NULL.  A row whose place is
  * MAXINT is skipped; of several rows with one place the last is written.  owner (with ids): n device ints, -1 before

@@ -1,5 +1,7 @@
 // Rows held in 8 bits: written, read back, scored against queries at listed ids, and the entry points.  The scan of a
 // range of rows is in vl_quant_scan.cu.
+#include <initializer_list>
+
 #include "vl_quant.cuh"
 
 namespace {
@@ -387,6 +389,15 @@ void launch_listed(const ListedArgs& a, int metric, cudaStream_t stream)
 }
 constexpr int kListedRounds = 96 * 16;       // columns up to which quant_listed_kernel rounds its queries itself
 
+// every place (null ones too) is aligned to elements of `size` bytes
+bool aligned(size_t size, std::initializer_list<const void*> places)
+{
+    uintptr_t bits = 0;
+    for (const void* p : places) bits |= (uintptr_t)p;
+    return bits % size == 0;
+}
+size_t type_size(int type) { return type == VL_TYPE_F32 ? 4 : 2; }
+
 #define VL_CHECK_SHAPE(name, n, dim, ld)                                                                                    \
     VL_CHECK_ARG((n) >= 0 && (n) < VL_MAXINT, name ": row count %lld outside int32", (long long)(n));                       \
     VL_CHECK_ARG((dim) > 0 && (dim) <= kMaxDim, name ": dimension %d outside 1..%d", (int)(dim), kMaxDim);                  \
@@ -405,7 +416,9 @@ extern "C" int vl_quant_write(const void* rows, int type, int64_t m, int dim, in
                  (long long)first_row, (long long)(first_row + m), (long long)n);
     if (m == 0) return 0;
     VL_CHECK_ARG(rows && status && (n == 0 || (codes && scales && norms && (!ids || owner))), "vl_quant_write: null pointer");
-    VL_CHECK_ARG((uintptr_t)codes % 16 == 0, "vl_quant_write: codes must be 16-byte aligned");
+    VL_CHECK_ARG(aligned(16, {codes}), "vl_quant_write: codes must be 16-byte aligned");
+    VL_CHECK_ARG(aligned(type_size(type), {rows}) && aligned(4, {ids, scales, norms, owner, status}),
+                 "vl_quant_write: a pointer is not aligned to its elements");
     const WriteArgs a = {rows, m, ld, dim, ids, first_row, codes, scales, norms, n, code_ld, owner, status};
     return write_any(a, type, (cudaStream_t)stream);
 }
@@ -420,7 +433,9 @@ extern "C" int vl_quant_read(const int8_t* codes, const float* scales, int64_t n
                  (long long)first_row, (long long)(first_row + m), (long long)n);
     if (m == 0) return 0;
     VL_CHECK_ARG(out && status && (n == 0 || (codes && scales)), "vl_quant_read: null pointer");
-    VL_CHECK_ARG((uintptr_t)codes % 16 == 0, "vl_quant_read: codes must be 16-byte aligned");
+    VL_CHECK_ARG(aligned(16, {codes}), "vl_quant_read: codes must be 16-byte aligned");
+    VL_CHECK_ARG(aligned(type_size(type), {out}) && aligned(4, {ids, scales, status}), "vl_quant_read: a pointer is not aligned to its elements");
+    VL_CHECK_ARG(out_ld >= dim || m == 1, "vl_quant_read: rows of the result overlap");
     const VlQuantRows held = {codes, scales, nullptr};
     const cudaStream_t s = (cudaStream_t)stream;
     if (type == VL_TYPE_F32) return read_rows<float>(held, n, dim, code_ld, ids, first_row, m, out, out_ld, status, s);
@@ -443,8 +458,9 @@ extern "C" int vl_quant_scores(const void* queries, int q_type, int64_t q_ld, in
     if (nq == 0 || row_lo == row_hi) return 0;
     const bool few = queries && nq <= VL_QUANT_FEW_QUERIES && code_ld <= VL_QUANT_FEW_COLUMNS;      // no need of the scratch
     VL_CHECK_ARG((few || (q_codes && q_scales && q_norms)) && codes && scales && norms && out && status, "vl_quant_scores: null pointer");
-    VL_CHECK_ARG(((uintptr_t)codes | (uintptr_t)q_codes) % 16 == 0, "vl_quant_scores: codes must be 16-byte aligned");
-    VL_CHECK_ARG((uintptr_t)out % (type == VL_TYPE_F32 ? 4 : 2) == 0, "vl_quant_scores: the result is not aligned to its elements");
+    VL_CHECK_ARG(aligned(16, {codes, q_codes}), "vl_quant_scores: codes must be 16-byte aligned");
+    VL_CHECK_ARG((!queries || aligned(type_size(q_type), {queries})) && aligned(type_size(type), {out}) &&
+                 aligned(4, {q_scales, q_norms, scales, norms, status}), "vl_quant_scores: a pointer is not aligned to its elements");
     VL_CHECK_ARG(out_ld >= row_hi - row_lo || nq == 1, "vl_quant_scores: rows of the result overlap");
     const cudaStream_t s = (cudaStream_t)stream;
     if (!few) {
@@ -467,7 +483,9 @@ extern "C" int vl_quant_listed(const void* queries, int q_type, int64_t q_ld, in
     if (nq == 0 || w == 0) return 0;
     const bool rounds = queries && code_ld <= kListedRounds;      // no need of the scratch
     VL_CHECK_ARG((rounds || (q_codes && q_scales && q_norms)) && ids && out && status && (n == 0 || (codes && scales && norms)), "vl_quant_listed: null pointer");
-    VL_CHECK_ARG(((uintptr_t)codes | (uintptr_t)q_codes) % 16 == 0, "vl_quant_listed: codes must be 16-byte aligned");
+    VL_CHECK_ARG(aligned(16, {codes, q_codes}), "vl_quant_listed: codes must be 16-byte aligned");
+    VL_CHECK_ARG((!queries || aligned(type_size(q_type), {queries})) && aligned(4, {q_scales, q_norms, scales, norms, ids, out, status}),
+                 "vl_quant_listed: a pointer is not aligned to its elements");
     const cudaStream_t s = (cudaStream_t)stream;
     if (!rounds) {
         const int rc = take_queries(queries, q_type, q_ld, nq, dim, code_ld, q_codes, q_scales, q_norms, status, s);
