@@ -199,7 +199,7 @@ int vl_knn_tile_parts(const uint16_t* rows_bf16, int64_t n, int dim_pad, const f
  * columns none for vl_quant_listed: NULL).  A wait inside the kernel that runs out sets VL_STATUS_TIMEOUT in *status.
  *
  * vl_quant_listed: out[b, j] = distance(queries[b], row ids[b, j]), MAXFLOAT where ids[b, j] == MAXINT (the counterpart
- * of vl_calculate_distances). */
+ * of vl_calculate_distances).  w <= 2^30. */
 #define VL_TYPE_F32 0
 #define VL_TYPE_BF16 1
 #define VL_TYPE_F16 2

@@ -387,6 +387,7 @@ void launch_listed(const ListedArgs& a, int metric, cudaStream_t stream)
     if (metric == VL_METRIC_COSINE) launch_listed<T, VL_METRIC_COSINE>(a, stream);
     else launch_listed<T, VL_METRIC_SQL2>(a, stream);
 }
+constexpr int kMaxList = 1 << 30;            // places of a list, and those 64 ahead that are asked for, are ints
 constexpr int kListedRounds = 96 * 16;       // columns up to which quant_listed_kernel rounds its queries itself
 
 // every place (null ones too) is aligned to elements of `size` bytes
@@ -477,7 +478,7 @@ extern "C" int vl_quant_listed(const void* queries, int q_type, int64_t q_ld, in
                                int code_ld, const int32_t* ids, int w, float* out, int metric, int* status, void* stream)
 {
     VL_CHECK_SHAPE("vl_quant_listed", n, dim, code_ld);
-    VL_CHECK_ARG(nq >= 0 && nq < VL_MAXINT && w >= 0, "vl_quant_listed: bad size");
+    VL_CHECK_ARG(nq >= 0 && nq < VL_MAXINT && w >= 0 && w <= kMaxList, "vl_quant_listed: bad size");
     VL_CHECK_ARG(!queries || (q_type >= VL_TYPE_F32 && q_type <= VL_TYPE_F16), "vl_quant_listed: unknown type %d", q_type);
     VL_CHECK_ARG(metric == VL_METRIC_COSINE || metric == VL_METRIC_SQL2, "vl_quant_listed: unknown metric %d", metric);
     if (nq == 0 || w == 0) return 0;

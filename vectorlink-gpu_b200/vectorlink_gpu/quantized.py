@@ -28,6 +28,7 @@ from .kernels import metric_code
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 PRODUCT = 2            # VL_QUANT_PRODUCT: the metric code of a plain product
 MAX_DIM = 131072       # 127^2 * dim has to fit 32 bits
+MAX_LIST = 1 << 30     # ids of one list
 LISTED_ROUNDS = 1536   # columns up to which the scoring of listed ids rounds its queries in registers
 FEW_QUERIES = (16, 4096)   # queries, and columns of them, up to which a scan rounds its queries itself
 FEW_ROWS = 64          # rows up to which a write to places is one launch
@@ -205,6 +206,8 @@ class QuantizedVectors:
         """`kernels.calculate_distances` over the held rows: out[i, j] = distance(queries[i], row beams[i, j]), MAXFLOAT
         where beams[i, j] == MAXINT."""
         (count, q, _alive) = self._queries(queries, MAXINT if self._columns <= LISTED_ROUNDS else 0)
+        # (the library takes a list's length as an int: a longer one would arrive cut to 32 bits)
+        assert beams.dim() == 2 and beams.size(1) <= MAX_LIST, f"list of up to {MAX_LIST} ids expected, got {tuple(beams.shape)}"
         beams = self._ids(beams, 2)
         (rows, width) = beams.shape
         assert rows == count
