@@ -193,7 +193,9 @@ int vl_knn_tile_parts(const uint16_t* rows_bf16, int64_t n, int dim_pad, const f
  * vl_quant_scores: out[b, r - row_lo] for every query b and every held row r in [row_lo, row_hi): metric
  * VL_QUANT_PRODUCT = s_b s_r <c_b, c_r> as any of the types; VL_METRIC_COSINE = (1 - product) / 2 clamped to [0, 1] and
  * VL_METRIC_SQL2 = |s_b c_b - s_r c_r|^2 as fp32.  <c_b, c_r> is summed exactly, the rest is combined in fp32, with
- * pairs of numbers where terms cancel (products of 16 bits are rounded from fp32); a pair has the same bits in every call.
+ * pairs of numbers where terms cancel, and squared distances below 2^-16 of |b|^2 + |r|^2 in 64 bits, so that those of near rows are
+ * exact to 2^-24 of themselves and those of equal rows are 0 (products of 16 bits are rounded from fp32); a pair has the
+ * same bits in every call.
  * queries [nq, dim] of q_type are held in 8 bits first, in q_codes [nq, code_ld], q_scales [nq], q_norms [nq]; with
  * queries == NULL these hold them already (up to 16 queries of up to 4096 columns need no such scratch, and up to 1536
  * columns none for vl_quant_listed: NULL).  A wait inside the kernel that runs out sets VL_STATUS_TIMEOUT in *status.

@@ -225,12 +225,15 @@ __device__ __forceinline__ void vl_quant_rows(const T* const (&x)[R], int dim, i
 // may be small against its terms:
 //   product  (qs cs) dot, two roundings
 //   cosine   1/2 - sh f, rounded once by an FMA, and that - sl f: two roundings of the result itself
-//   l2       (a - t) + (b - t): of near rows both are small as well.  a - sh f and b - sh f are rounded once, the low parts
-//            of a, b and t (each below 2^-22 of its number) are summed apart
-// Scales within 2^+-40 keep every term a normal number and the pairs exact.  Other rows take 64-bit arithmetic, whose
-// conversions run at 4 a clock and SM (all results in 64 bits: 500 M distances 1,039 us, now 600).
+//   l2       squared lengths a, b are pairs hi - over as well, hi of 20 bits, so that of rows of like length their sum is exact
+//            (otherwise its error is made exactly and summed with the rest).  2 sh f is taken from it in one FMA, and the rest
+//            (below 2^-18 (a + b), summed apart) is added: two roundings of the result itself, and 5 * 2^-43 (a + b).  In results
+//            below 2^-16 (a + b) that would show, and near rows are made from the differences of their codes and scales
+//            instead: vl_quant_pair64.
+// Scales within 2^+-40 keep every term a normal number and the pairs exact.  Other rows take 64-bit arithmetic too, whose
+// conversions run at 4 a clock and SM.
 struct VlQuantSide {
-    float s, hi, lo;         // scale; squared length (squared l2 only) as a pair of numbers
+    float s, hi, over;       // scale; squared length (squared l2 only): hi - over
     int n;
     bool ordinary;
 };
@@ -244,61 +247,98 @@ __device__ __forceinline__ VlQuantSide vl_quant_side(float s, int n)
     VlQuantSide r = {s, 0.0f, 0.0f, n, vl_quant_ordinary(s, n)};
     if (METRIC == VL_METRIC_SQL2) {
         const float sh = __fmul_rn(s, s), sl = __fmaf_rn(s, s, -sh), f = (float)n;
-        r.hi = __fmul_rn(sh, f);
-        r.lo = __fmaf_rn(sl, f, __fmaf_rn(sh, f, -r.hi));
+        const float length = __fmul_rn(sh, f);
+        r.hi = __uint_as_float(__float_as_uint(length) & ~15u);
+        r.over = __fadd_rn(__fsub_rn(r.hi, length), __fmaf_rn(-sl, f, __fmaf_rn(-sh, f, length)));
     }
     return r;
 }
+// The part of a + b below which a squared distance is that of near rows.
+constexpr float kQuantNear = 1.0f / (1 << 16);
+
+// In 64 bits, for any rows.  Products of scales are exact here.  l2 with D = codes_q - codes_r is
+//   |qs c_q - cs c_r|^2 = (qs - cs)^2 dot + qs^2 <c_q, D> - cs^2 <c_r, D>,   <c_q, D> = qn - dot, <c_r, D> = dot - cn,
+// whole numbers that are small for near rows, as is the difference of their scales: nothing large cancels, and equal rows are
+// exactly 0 apart.
 template <int METRIC>
+__device__ __forceinline__ float vl_quant_pair64(int dot, float qs, int qn, float cs, int cn)
+{
+    const double q = qs, c = cs, f = dot;
+    if (METRIC == VL_METRIC_SQL2) {
+        const double apart = __dsub_rn(q, c);
+        const double a = __dmul_rn(__dmul_rn(q, q), __dsub_rn((double)qn, f)), b = __dmul_rn(__dmul_rn(c, c), __dsub_rn((double)cn, f));
+        const float d = (float)__fma_rn(__dmul_rn(apart, apart), f, __dadd_rn(a, b));
+        return d <= 0.0f ? 0.0f : d;                        // a NaN stays
+    }
+    const double t = __dmul_rn(__dmul_rn(q, c), f);
+    if (METRIC == VL_QUANT_PRODUCT) return (float)t;
+    const float d = (float)__dmul_rn(__dsub_rn(1.0, t), 0.5);
+    return d <= 0.0f ? 0.0f : (d > 1.0f ? 1.0f : d);
+}
+template <int METRIC>
+static __device__ __noinline__ float vl_quant_pair64_apart(int dot, float qs, int qn, float cs, int cn)
+{
+    return vl_quant_pair64<METRIC>(dot, qs, qn, cs, cn);
+}
+// APART: what is rarely taken stands apart, and leaves the caller its registers (30,000 lists of 64 ids, 1M x 768, l2: 262 us, and
+// 274 with it inside).
+template <int METRIC, bool APART>
 __device__ __forceinline__ float vl_quant_pair(int dot, const VlQuantSide& q, const VlQuantSide& r)
 {
     if (q.ordinary && r.ordinary) {
         const float f = (float)dot;
         if (METRIC == VL_QUANT_PRODUCT) return __fmul_rn(__fmul_rn(q.s, r.s), f);
-        const float cs = METRIC == VL_METRIC_COSINE ? 0.5f * r.s : r.s;
-        const float sh = __fmul_rn(q.s, cs), rest = __fmaf_rn(-q.s, cs, sh);          // rest = -sl
-        if (METRIC == VL_METRIC_COSINE) return __saturatef(__fmaf_rn(rest, f, __fmaf_rn(-sh, f, 0.5f)));
-        const float u = __fadd_rn(__fmaf_rn(-sh, f, q.hi), __fmaf_rn(-sh, f, r.hi));
-        return fmaxf(__fadd_rn(u, __fmaf_rn(__fadd_rn(rest, rest), f, __fadd_rn(q.lo, r.lo))), 0.0f);
+        const float cs = METRIC == VL_METRIC_COSINE ? 0.5f * r.s : 2.0f * r.s;
+        const float sh = __fmul_rn(q.s, cs), sl = __fmaf_rn(q.s, cs, -sh);
+        if (METRIC == VL_METRIC_COSINE) return __saturatef(__fmaf_rn(-sl, f, __fmaf_rn(-sh, f, 0.5f)));
+        const float ab = __fadd_rn(q.hi, r.hi), of_r = __fsub_rn(ab, q.hi);
+        const float more = __fadd_rn(__fsub_rn(__fsub_rn(ab, of_r), q.hi), __fsub_rn(of_r, r.hi));           // ab - a - b, exactly
+        const float d = __fsub_rn(__fmaf_rn(-sh, f, ab), __fmaf_rn(sl, f, __fadd_rn(__fadd_rn(q.over, r.over), more)));
+        if (d > __fmul_rn(kQuantNear, ab)) return d;
     }
-    const double t = __dmul_rn(__dmul_rn((double)q.s, (double)r.s), (double)dot);
-    if (METRIC == VL_QUANT_PRODUCT) return (float)t;
-    if (METRIC == VL_METRIC_COSINE) {
-        const float d = (float)__dmul_rn(__dsub_rn(1.0, t), 0.5);
-        return d <= 0.0f ? 0.0f : (d > 1.0f ? 1.0f : d);    // a NaN stays
-    }
-    const double a = __dmul_rn(__dmul_rn((double)q.s, (double)q.s), (double)q.n);
-    const double b = __dmul_rn(__dmul_rn((double)r.s, (double)r.s), (double)r.n);
-    const float d = (float)__fma_rn(-2.0, t, __dadd_rn(a, b));        // 2 t is exact
-    return d <= 0.0f ? 0.0f : d;
+    return APART ? vl_quant_pair64_apart<METRIC>(dot, q.s, q.n, r.s, r.n) : vl_quant_pair64<METRIC>(dot, q.s, q.n, r.s, r.n);
 }
 
-// Two results at once of ordinary rows, by the operations of vl_quant_pair on packed numbers: `s`, `hi`, `lo` of two
-// queries, and of the held row its (for cosine halved) scale, the negative of that, and its squared length.
-template <int METRIC>
-__device__ __forceinline__ void vl_quant_pair2(int dot0, int dot1, vl_f2 s, vl_f2 hi, vl_f2 lo, vl_f2 cs, vl_f2 ncs, vl_f2 rhi, vl_f2 rlo,
-                                               float& r0, float& r1)
+// Whether 24 bits hold the sum of any two numbers of 20 bits from `less` to `more`: leading digits three places apart, a carry, and 20.
+__device__ __forceinline__ bool vl_quant_alike(float less, float more)
+{
+    return (int)(__float_as_uint(more) >> 23) - (int)(__float_as_uint(less) >> 23) <= 3;
+}
+
+// Two results at once of ordinary rows, by the operations of vl_quant_pair on packed numbers: `s`, `hi`, `over` of two
+// queries, and of the held row its scale (for cosine half of it, for l2 twice), the negative of that, and its squared length.
+// ALIKE: a + b is exact, and all are at most 16 times the shortest one.  `least` takes the smallest squared distance, or the smallest
+// excess over that of near rows where lengths vary: where it is not above that of near rows, or not above 0, vl_quant_pair has to look at them.
+template <int METRIC, bool ALIKE>
+__device__ __forceinline__ void vl_quant_pair2(int dot0, int dot1, vl_f2 s, vl_f2 hi, vl_f2 over, vl_f2 cs, vl_f2 ncs, vl_f2 rhi, vl_f2 rover,
+                                               float& r0, float& r1, float& least)
 {
     const vl_f2 f = vl_f2_pack((float)dot0, (float)dot1);
-    const vl_f2 sh = vl_f2_mul(s, cs);
     if (METRIC == VL_QUANT_PRODUCT) {
-        vl_f2_unpack(vl_f2_mul(sh, f), r0, r1);
+        vl_f2_unpack(vl_f2_mul(vl_f2_mul(s, cs), f), r0, r1);
         return;
     }
-    const vl_f2 nsh = vl_f2_mul(s, ncs), rest = vl_f2_fma(s, ncs, sh);
+    const vl_f2 nsh = vl_f2_mul(s, ncs);
     if (METRIC == VL_METRIC_COSINE) {
-        const vl_f2 h = vl_f2_fma(nsh, f, vl_f2_pack(0.5f, 0.5f));
+        const vl_f2 h = vl_f2_fma(nsh, f, vl_f2_pack(0.5f, 0.5f)), nsl = vl_f2_fma(s, ncs, vl_f2_mul(s, cs));
         float f0, f1, h0, h1, l0, l1;
         vl_f2_unpack(f, f0, f1);
         vl_f2_unpack(h, h0, h1);
-        vl_f2_unpack(rest, l0, l1);
+        vl_f2_unpack(nsl, l0, l1);
         r0 = __saturatef(__fmaf_rn(l0, f0, h0));
         r1 = __saturatef(__fmaf_rn(l1, f1, h1));
     } else {
-        const vl_f2 u = vl_f2_add(vl_f2_fma(nsh, f, hi), vl_f2_fma(nsh, f, rhi));
-        vl_f2_unpack(vl_f2_add(u, vl_f2_fma(vl_f2_add(rest, rest), f, vl_f2_add(lo, rlo))), r0, r1);
-        r0 = fmaxf(r0, 0.0f);
-        r1 = fmaxf(r1, 0.0f);
+        const vl_f2 ab = vl_f2_add(hi, rhi), sl = vl_f2_fma(s, cs, nsh);
+        vl_f2 rest = vl_f2_add(over, rover);
+        if (!ALIKE) {
+            const vl_f2 of_r = vl_f2_sub(ab, hi);
+            rest = vl_f2_add(rest, vl_f2_add(vl_f2_sub(vl_f2_sub(ab, of_r), hi), vl_f2_sub(of_r, rhi)));
+        }
+        const vl_f2 d = vl_f2_sub(vl_f2_fma(nsh, f, ab), vl_f2_fma(sl, f, rest));
+        vl_f2_unpack(d, r0, r1);
+        float l0, l1;
+        vl_f2_unpack(ALIKE ? d : vl_f2_fma(vl_f2_pack(-kQuantNear, -kQuantNear), ab, d), l0, l1);
+        asm("min.f32 %0, %1, %2, %3;" : "=f"(least) : "f"(l0), "f"(l1), "f"(least));
     }
 }
 

@@ -35,7 +35,7 @@ constexpr uint32_t kTmemCols = 2 * kMaxQueries;
 constexpr uint32_t kStageRow = kTileRows * 4 + 15;
 constexpr uint32_t kStageBytes = (kChunk * kStageRow + 16 + 127) & ~127u;
 
-// shared memory behind the 1024-byte aligned base: barriers, the block's queries (scales, squared lengths (hi, lo), squared
+// shared memory behind the 1024-byte aligned base: barriers, the block's queries (scales, squared lengths (hi, over), squared
 // sums), the finishing groups' buffers; the operands come first
 constexpr uint32_t kTailBytes = (8 * (2 * kMaxStages + 2 * kMaxAccs + 3) + 8 + 127) & ~127u;
 constexpr uint32_t kOperandBytes = (227 * 1024 - 1024 - kTailBytes - kMaxQueries * 16 - kParts * kStageBytes) & ~1023u;
@@ -194,6 +194,40 @@ static __device__ __noinline__ void hold_query(const ScanArgs& a, int b, unsigne
     }
 }
 
+// A lane's results of a chunk: 16 queries' values are read four at a time, since shared memory feeds the products too.
+template <int METRIC, bool ALIKE>
+__device__ __forceinline__ void finish_chunk(const uint32_t (&v)[kChunk], const float* q_scale, vl_f2 cs, vl_f2 ncs, vl_f2 hi, vl_f2 over,
+                                             float (&r)[kChunk], float& least)
+{
+#pragma unroll
+    for (int j = 0; j < kChunk; j += 4) {
+        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(q_scale + j);
+        ulonglong2 q_hi = {0ull, 0ull}, q_over = {0ull, 0ull};
+        if (METRIC == VL_METRIC_SQL2) {
+            q_hi = *reinterpret_cast<const ulonglong2*>(q_scale + kMaxQueries + j);
+            q_over = *reinterpret_cast<const ulonglong2*>(q_scale + 2 * kMaxQueries + j);
+        }
+        vl_quant_pair2<METRIC, ALIKE>((int)v[j], (int)v[j + 1], s.x, q_hi.x, q_over.x, cs, ncs, hi, over, r[j], r[j + 1], least);
+        vl_quant_pair2<METRIC, ALIKE>((int)v[j + 2], (int)v[j + 3], s.y, q_hi.y, q_over.y, cs, ncs, hi, over, r[j + 2], r[j + 3], least);
+    }
+}
+// ... one by one: rows that are not ordinary, and near rows among others
+template <int METRIC>
+__device__ __forceinline__ float finish_pair(int dot, const float* q_scale, const VlQuantSide& held)
+{
+    const int n = *reinterpret_cast<const int*>(q_scale + 3 * kMaxQueries);
+    const VlQuantSide q = {*q_scale, q_scale[kMaxQueries], q_scale[2 * kMaxQueries], n, vl_quant_ordinary(*q_scale, n)};
+    return vl_quant_pair<METRIC, false>(dot, q, held);
+}
+// ... and put over those in the buffer.  Not inlined: near rows are rare, and the loop over chunks has the registers for itself.
+static __device__ __noinline__ void finish_near(int4 d0, int4 d1, int4 d2, int4 d3, const float* q_scale, float row_scale, int row_n, uint32_t at, uint32_t pitch)
+{
+    const VlQuantSide held = vl_quant_side<VL_METRIC_SQL2>(row_scale, row_n);
+    const int dots[kChunk] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w, d2.x, d2.y, d2.z, d2.w, d3.x, d3.y, d3.z, d3.w};
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) st_shared<float>(at + j * pitch, finish_pair<VL_METRIC_SQL2>(dots[j], q_scale + j, held));
+}
+
 template <typename T, int METRIC, bool RESIDENT, bool SECTORS>
 __global__ void __launch_bounds__(kThreads, 1)
 quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ ScanArgs a)
@@ -334,8 +368,8 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
         const int64_t ld_bytes = a.out_ld * (int64_t)sizeof(T);
         float* q_scale = reinterpret_cast<float*>(base_ptr + kOffQueries);
         float* q_hi = q_scale + kMaxQueries;
-        float* q_lo = q_hi + kMaxQueries;
-        int* q_n = reinterpret_cast<int*>(q_lo + kMaxQueries);
+        float* q_over = q_hi + kMaxQueries;
+        int* q_n = reinterpret_cast<int*>(q_over + kMaxQueries);
         const uint32_t stage = base + kOffStage + group * kStageBytes;
         const uint32_t pitch = kTileRows * sizeof(T) + (SECTORS ? 0u : (uint32_t)ld_bytes & 15u);
         uint32_t buf = way, tph = 0;
@@ -360,8 +394,8 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
             barrier_sync(1, 32 * kFinishWarps);
             auto keep = [&](int i, const VlQuantSide& q) {
                 q_scale[i] = q.s;
-                q_hi[i] = q.hi;
-                q_lo[i] = q.lo;
+                q_hi[i] = i < here ? q.hi : __int_as_float(0x7f800000);         // padding is near no row
+                q_over[i] = q.over;
                 q_n[i] = q.n;
             };
             if (RESIDENT && a.queries) {                            // one block, one warp for each of its 16 queries
@@ -380,8 +414,17 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
             }
             barrier_sync(1, 32 * kFinishWarps);
             bool plain = true;
-            for (int i = lane; i < a.nb; i += 32) plain = plain && vl_quant_ordinary(q_scale[i], q_n[i]);
+            uint32_t most = 0u, some = 0x7f7fffffu;                 // bits of the queries' largest squared length and the smallest one but 0
+            for (int i = lane; i < here; i += 32) {
+                plain = plain && vl_quant_ordinary(q_scale[i], q_n[i]);
+                if (METRIC == VL_METRIC_SQL2) {
+                    const uint32_t bits = __float_as_uint(q_hi[i]);
+                    most = max(most, bits);
+                    if (bits) some = min(some, bits);
+                }
+            }
             plain = __all_sync(0xffffffffu, plain);
+            const float q_most = __uint_as_float(__reduce_max_sync(0xffffffffu, most)), q_least = __uint_as_float(__reduce_min_sync(0xffffffffu, some));
             float next_cs;
             int next_cn;
             fetch(rt0 + first * a.groups, next_cs, next_cn);
@@ -395,51 +438,38 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * a.nb;
                 const bool fast = plain && __all_sync(0xffffffffu, held.ordinary);
-                const float cs = METRIC == VL_METRIC_COSINE ? 0.5f * held.s : held.s;
-                const vl_f2 cs2 = vl_f2_pack(cs, cs), ncs2 = vl_f2_pack(-cs, -cs);
-                const vl_f2 hi2 = vl_f2_pack(held.hi, held.hi), lo2 = vl_f2_pack(held.lo, held.lo);
+                const float cs = METRIC == VL_METRIC_COSINE ? 0.5f * held.s : (METRIC == VL_METRIC_SQL2 ? 2.0f * held.s : held.s);
+                const vl_f2 cs2 = vl_f2_pack(cs, cs), ncs2 = vl_f2_pack(-cs, -cs), over2 = vl_f2_pack(held.over, held.over), hi2 = vl_f2_pack(held.hi, held.hi);
+                const bool alike = METRIC != VL_METRIC_SQL2 || __all_sync(0xffffffffu, held.hi == 0.0f || vl_quant_alike(fminf(q_least, held.hi), fmaxf(q_most, held.hi)));
+                const float near = alike ? __fmul_rn(kQuantNear, __fadd_rn(q_most, held.hi)) : 0.0f;          // that of no pair is larger
                 const bool edge = !SECTORS && rt == 0 || rt + 1 == row_tiles;
                 char* out = reinterpret_cast<char*>(a.out) + (b0 + part * kChunk) * ld_bytes;
                 const uint32_t mine = stage + (quarter * 32 + lane) * (uint32_t)sizeof(T);
 #pragma unroll 1
                 for (int c0 = part * kChunk; c0 < a.nb; c0 += a.parts * kChunk, out += a.parts * kChunk * ld_bytes) {
                     const uint32_t off = SECTORS ? 0u : (uint32_t)(uintptr_t)out & 15u;
-                    uint32_t v[kChunk];                             // columns behind nb: of the next accumulator, or of none, and not stored
+                    uint32_t v[kChunk];
                     tc_load(taddr + c0, v);
                     tc_wait_ld();
-                    const float* qs = q_scale + c0;
                     if (c0 + a.parts * kChunk >= a.nb) {            // the tile's last columns are in registers
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
                     }
-                    if (fast) {
-#pragma unroll
-                        for (int j = 0; j < kChunk; j += 4) {       // four queries' values in one access each: shared memory feeds the products too
-                            const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(qs + j);
-                            ulonglong2 hi = {0ull, 0ull}, lo = {0ull, 0ull};
-                            if (METRIC == VL_METRIC_SQL2) {
-                                hi = *reinterpret_cast<const ulonglong2*>(qs + kMaxQueries + j);
-                                lo = *reinterpret_cast<const ulonglong2*>(qs + 2 * kMaxQueries + j);
-                            }
-                            float r0, r1, r2, r3;
-                            vl_quant_pair2<METRIC>((int)v[j], (int)v[j + 1], s.x, hi.x, lo.x, cs2, ncs2, hi2, lo2, r0, r1);
-                            vl_quant_pair2<METRIC>((int)v[j + 2], (int)v[j + 3], s.y, hi.y, lo.y, cs2, ncs2, hi2, lo2, r2, r3);
-                            v[j] = __float_as_uint(r0);
-                            v[j + 1] = __float_as_uint(r1);
-                            v[j + 2] = __float_as_uint(r2);
-                            v[j + 3] = __float_as_uint(r3);
-                        }
+                    float r[kChunk], least = __int_as_float(0x7f800000);
+                    if (fast && alike) {
+                        finish_chunk<METRIC, true>(v, q_scale + c0, cs2, ncs2, hi2, over2, r, least);
+                    } else if (fast) {
+                        finish_chunk<METRIC, false>(v, q_scale + c0, cs2, ncs2, hi2, over2, r, least);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < kChunk; ++j) {
-                            const int i = c0 + j;
-                            const VlQuantSide q = {q_scale[i], q_hi[i], q_lo[i], q_n[i], vl_quant_ordinary(q_scale[i], q_n[i])};
-                            v[j] = __float_as_uint(vl_quant_pair<METRIC>((int)v[j], q, held));
-                        }
+                        for (int j = 0; j < kChunk; ++j) r[j] = finish_pair<METRIC>((int)v[j], q_scale + c0 + j, held);
                     }
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) st_shared<T>(mine + off + j * pitch, __uint_as_float(v[j]));
+                    for (int j = 0; j < kChunk; ++j) st_shared<T>(mine + off + j * pitch, r[j]);
+                    if (METRIC == VL_METRIC_SQL2 && least <= near)
+                        finish_near(make_int4(v[0], v[1], v[2], v[3]), make_int4(v[4], v[5], v[6], v[7]), make_int4(v[8], v[9], v[10], v[11]),
+                                    make_int4(v[12], v[13], v[14], v[15]), q_scale + c0, held.s, held.n, mine + off, pitch);
                     barrier_sync(2 + group, 128);
                     const int left = here - c0 < kChunk ? here - c0 : kChunk;
                     if (edge) store_rows_edge<T>(out, ld_bytes, left, rt, rt + 1 == row_tiles, count, a.step, a.lead, base_ptr + (stage - base) + off, pitch, in_group);
