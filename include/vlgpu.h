@@ -198,7 +198,8 @@ int vl_knn_tile_parts(const uint16_t* rows_bf16, int64_t n, int dim_pad, const f
  * same bits in every call.
  * queries [nq, dim] of q_type are held in 8 bits first, in q_codes [nq, code_ld], q_scales [nq], q_norms [nq]; with
  * queries == NULL these hold them already (up to 16 queries of up to 4096 columns need no such scratch, and up to 1536
- * columns none for vl_quant_listed: NULL).  A wait inside the kernel that runs out sets VL_STATUS_TIMEOUT in *status.
+ * columns none for vl_quant_listed: NULL).  A wait inside the kernel that runs out sets VL_STATUS_TIMEOUT in *status,
+ * and what is not made by then becomes NaN.  vl_quant_scores_wait takes the longest such wait in microseconds (0: two seconds).
  *
  * vl_quant_listed: out[b, j] = distance(queries[b], row ids[b, j]), MAXFLOAT where ids[b, j] == MAXINT (the counterpart
  * of vl_calculate_distances).  w <= 2^30. */
@@ -215,6 +216,10 @@ int vl_quant_scores(const void* queries, int q_type, int64_t q_ld, int8_t* q_cod
                     int64_t nq, const int8_t* codes, const float* scales, const int32_t* norms, int64_t n, int dim,
                     int code_ld, int64_t row_lo, int64_t row_hi, void* out, int type, int64_t out_ld, int metric,
                     int* status, void* stream);
+int vl_quant_scores_wait(const void* queries, int q_type, int64_t q_ld, int8_t* q_codes, float* q_scales, int32_t* q_norms,
+                         int64_t nq, const int8_t* codes, const float* scales, const int32_t* norms, int64_t n, int dim,
+                         int code_ld, int64_t row_lo, int64_t row_hi, void* out, int type, int64_t out_ld, int metric,
+                         int wait_us, int* status, void* stream);
 int vl_quant_listed(const void* queries, int q_type, int64_t q_ld, int8_t* q_codes, float* q_scales, int32_t* q_norms,
                     int64_t nq, const int8_t* codes, const float* scales, const int32_t* norms, int64_t n, int dim,
                     int code_ld, const int32_t* ids, int w, float* out, int metric, int* status, void* stream);

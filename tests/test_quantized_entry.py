@@ -64,3 +64,9 @@ def test_rows_of_a_result_that_overlap(built_lib):
         assert "overlap" in refusal("vl_quant_read", READ, out_ld=out_ld)
     for out_ld in (9, 0, -10):
         assert "overlap" in refusal("vl_quant_scores", SCORES, out_ld=out_ld)
+
+
+def test_a_negative_wait(built_lib):
+    wait = {**{k: v for k, v in SCORES.items() if k not in ("status", "stream")}, "wait_us": 0, "status": 256, "stream": None}
+    assert "wait" in refusal("vl_quant_scores_wait", wait, wait_us=-1)
+    assert "aligned" in refusal("vl_quant_scores_wait", wait, out=258)

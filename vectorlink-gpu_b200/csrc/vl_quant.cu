@@ -449,8 +449,18 @@ extern "C" int vl_quant_scores(const void* queries, int q_type, int64_t q_ld, in
                                int code_ld, int64_t row_lo, int64_t row_hi, void* out, int type, int64_t out_ld, int metric,
                                int* status, void* stream)
 {
+    return vl_quant_scores_wait(queries, q_type, q_ld, q_codes, q_scales, q_norms, nq, codes, scales, norms, n, dim, code_ld, row_lo, row_hi, out, type,
+                                out_ld, metric, 0, status, stream);
+}
+
+extern "C" int vl_quant_scores_wait(const void* queries, int q_type, int64_t q_ld, int8_t* q_codes, float* q_scales, int32_t* q_norms,
+                                    int64_t nq, const int8_t* codes, const float* scales, const int32_t* norms, int64_t n, int dim,
+                                    int code_ld, int64_t row_lo, int64_t row_hi, void* out, int type, int64_t out_ld, int metric,
+                                    int wait_us, int* status, void* stream)
+{
     VL_CHECK_SHAPE("vl_quant_scores", n, dim, code_ld);
     VL_CHECK_ARG(nq >= 0 && nq < VL_MAXINT, "vl_quant_scores: bad size");
+    VL_CHECK_ARG(wait_us >= 0, "vl_quant_scores: a wait of %d microseconds", wait_us);
     VL_CHECK_ARG(0 <= row_lo && row_lo <= row_hi && row_hi <= n, "vl_quant_scores: bad row range");
     VL_CHECK_ARG(!queries || (q_type >= VL_TYPE_F32 && q_type <= VL_TYPE_F16), "vl_quant_scores: unknown type %d", q_type);
     VL_CHECK_ARG(metric == VL_METRIC_COSINE || metric == VL_METRIC_SQL2 || metric == VL_QUANT_PRODUCT, "vl_quant_scores: unknown metric %d", metric);
@@ -470,7 +480,7 @@ extern "C" int vl_quant_scores(const void* queries, int q_type, int64_t q_ld, in
         queries = nullptr;
     }
     return vl_quant_scan(queries, q_type, q_ld, {q_codes, q_scales, q_norms}, nq, {codes, scales, norms}, n, dim, code_ld, row_lo, row_hi, out,
-                         type, out_ld, metric, status, s);
+                         type, out_ld, metric, wait_us, status, s);
 }
 
 extern "C" int vl_quant_listed(const void* queries, int q_type, int64_t q_ld, int8_t* q_codes, float* q_scales, int32_t* q_norms,

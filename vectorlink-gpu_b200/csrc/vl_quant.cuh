@@ -347,7 +347,7 @@ __device__ __forceinline__ void vl_quant_pair2(int dot0, int dot1, vl_f2 s, vl_f
 #define VL_QUANT_FEW_COLUMNS 4096
 
 // Scores of every query against the rows [row_lo, row_hi) (vl_quant_scan.cu); codes of both are 16-byte aligned.  `queries`:
-// few floating-point rows that the scan holds in 8 bits itself, or null: `q` has them.
+// few floating-point rows that the scan holds in 8 bits itself, or null: `q` has them.  `wait_us`: the longest wait inside, 0 for two seconds.
 int vl_quant_scan(const void* queries, int q_type, int64_t q_ld, const VlQuantRows& q, int64_t nq, const VlQuantRows& rows, int64_t n,
-                  int dim, int code_ld, int64_t row_lo, int64_t row_hi, void* out, int type, int64_t out_ld, int metric, int* status,
+                  int dim, int code_ld, int64_t row_lo, int64_t row_hi, void* out, int type, int64_t out_ld, int metric, int wait_us, int* status,
                   cudaStream_t stream);

@@ -8,7 +8,8 @@
 //                      ring in shared memory.  The queries of a CTA's block stay in shared memory where they fit.
 //   warp 1           : issues the products into one of the accumulators
 //   warps 2..17      : four groups that finish the scores of an accumulator each and store them
-// Waits are bounded; a wait that runs out sets VL_STATUS_TIMEOUT and ends all roles (vl_tensor.cuh).
+// Waits are bounded; a wait that runs out sets VL_STATUS_TIMEOUT and ends all roles of its CTA (vl_tensor.cuh), whose results
+// that are not made by then become NaN.
 #include "vl_quant.cuh"
 #include "vl_tensor.cuh"
 
@@ -42,7 +43,9 @@ constexpr uint32_t kOperandBytes = (227 * 1024 - 1024 - kTailBytes - kMaxQueries
 constexpr uint32_t kOffBars = kOperandBytes;
 constexpr uint32_t kOffSlot = kOffBars + 8 * (2 * kMaxStages + 2 * kMaxAccs + 3);
 constexpr uint32_t kOffAbort = kOffSlot + 4;
+constexpr uint32_t kOffStop = kOffAbort + 4;
 constexpr uint32_t kOffQueries = kOffBars + kTailBytes;
+static_assert(kOffStop + 8 * kParts <= kOffQueries, "two words for each finishing group");
 constexpr uint32_t kOffStage = kOffQueries + kMaxQueries * 16;
 constexpr uint32_t kSmemBytes = kOffStage + kParts * kStageBytes + 1024;   // + slack for the alignment
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
@@ -67,6 +70,7 @@ struct ScanArgs {
     void* out;
     int64_t out_ld;
     int* status;
+    int wait_us;                   // longest wait for another role
 };
 
 // D[tmem] (+)= A[smem] * B[smem]^T, int8 inputs, int32 accumulate
@@ -159,6 +163,37 @@ __device__ __noinline__ void store_rows_edge(char* out, int64_t ld_bytes, int le
         for (int64_t e = lo + (thread & 7); e < from; e += 8) o[e] = row[e];
         for (int64_t e = from + (thread & 7) * kWide; e < to; e += 8 * kWide) *reinterpret_cast<int4*>(o + e) = *reinterpret_cast<const int4*>(row + e);
         for (int64_t e = to + (thread & 7); e < hi; e += 8) o[e] = row[e];
+    }
+}
+
+// The first of a block's tiles that a way finishes, `behind` tiles after the CTA's first: tiles are dealt to the ways in turn, across blocks.
+__device__ __forceinline__ int64_t first_tile(int way, int64_t behind, int ways) { return (way - behind % ways + ways) % ways; }
+
+// NaN as the results that a group has not made when its wait ran out: tile rt of block qb, and what comes after it.
+template <typename T, bool SECTORS>
+__device__ __noinline__ void store_none(const ScanArgs& a, unsigned char* stage, int qb, int64_t rt, int way, int part, int thread, int barrier)
+{
+    const int64_t count = a.row_hi - a.row_lo, row_tiles = (count + a.step - 1) / a.step, ld_bytes = a.out_ld * (int64_t)sizeof(T);
+    const int qb0 = blockIdx.x / a.groups, qb_step = gridDim.x / a.groups, rt0 = blockIdx.x % a.groups, ways = kParts / a.parts;
+    const int64_t mine = rt0 < row_tiles ? (row_tiles - rt0 + a.groups - 1) / a.groups : 0;
+    const uint32_t pitch = kTileRows * sizeof(T) + (SECTORS ? 0u : (uint32_t)ld_bytes & 15u);
+    for (int i = thread * 4; i < (int)kStageBytes; i += 128 * 4) *reinterpret_cast<uint32_t*>(stage + i) = 0xffffffffu;        // in every type
+    barrier_sync(barrier, 128);
+#pragma unroll 1
+    while (qb < a.qblocks) {
+        const int64_t b0 = (int64_t)qb * a.nb;
+        const int here = a.nq - b0 < a.nb ? (int)(a.nq - b0) : a.nb;
+#pragma unroll 1
+        for (; rt < row_tiles; rt += (int64_t)ways * a.groups) {
+#pragma unroll 1
+            for (int c0 = part * kChunk; c0 < here; c0 += a.parts * kChunk) {
+                char* out = reinterpret_cast<char*>(a.out) + (b0 + c0) * ld_bytes;
+                const uint32_t off = SECTORS ? 0u : (uint32_t)(uintptr_t)out & 15u;
+                store_rows_edge<T>(out, ld_bytes, here - c0 < kChunk ? here - c0 : kChunk, rt, rt + 1 == row_tiles, count, a.step, a.lead, stage + off, pitch, thread);
+            }
+        }
+        qb += qb_step;
+        rt = rt0 + first_tile(way, (qb - qb0) / qb_step * mine, ways) * a.groups;
     }
 }
 
@@ -278,7 +313,7 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
 #pragma unroll 1
         for (int qb = qb0; qb < a.qblocks && ok; qb += qb_step) {
             if (RESIDENT && !a.queries) {
-                ok = mbar_wait(bar_q_empty, (nres & 1u) ^ 1u, abort_flag, a.status);
+                ok = mbar_wait(bar_q_empty, (nres & 1u) ^ 1u, abort_flag, a.status, a.wait_us);
                 if (!ok) break;
                 ++nres;
                 mbar_expect_tx(bar_q_full, a.kblocks * q_bytes);
@@ -289,7 +324,7 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
                 const int y = (int)(a.row_lo + rt * a.step - a.lead);        // rows before the first one arrive as zeros, or are not stored
 #pragma unroll 1
                 for (int kb = 0; kb < a.kblocks; ++kb) {
-                    ok = mbar_wait(bar_empty + 8 * s, ph ^ 1u, abort_flag, a.status);
+                    ok = mbar_wait(bar_empty + 8 * s, ph ^ 1u, abort_flag, a.status, a.wait_us);
                     if (!ok) break;
                     mbar_expect_tx(bar_full + 8 * s, a.stage_bytes);
                     tma_load_2d(ring + s * a.stage_bytes, &tmap_rows, kb * kBlockK, y, bar_full + 8 * s);
@@ -321,19 +356,19 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
 #pragma unroll 1
         for (int qb = qb0; qb < a.qblocks && ok; qb += qb_step) {
             if (RESIDENT) {
-                ok = __all_sync(0xffffffffu, mbar_wait(bar_q_full, nres & 1u, abort_flag, a.status));
+                ok = __all_sync(0xffffffffu, mbar_wait(bar_q_full, nres & 1u, abort_flag, a.status, a.wait_us));
                 if (!ok) break;
                 ++nres;
             }
 #pragma unroll 1
             for (int64_t rt = rt0; rt < row_tiles && ok; rt += a.groups) {
-                ok = __all_sync(0xffffffffu, mbar_wait(bar_tempty + 8 * buf, tph ^ 1u, abort_flag, a.status));
+                ok = __all_sync(0xffffffffu, mbar_wait(bar_tempty + 8 * buf, tph ^ 1u, abort_flag, a.status, a.wait_us));
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + buf * a.nb;
 #pragma unroll 1
                 for (int kb = 0; kb < a.kblocks; ++kb) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(bar_full + 8 * s, ph, abort_flag, a.status));
+                    ok = __all_sync(0xffffffffu, mbar_wait(bar_full + 8 * s, ph, abort_flag, a.status, a.wait_us));
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t a_desc = smem_desc_sw128(ring + s * a.stage_bytes);
@@ -371,6 +406,7 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
         float* q_over = q_hi + kMaxQueries;
         int* q_n = reinterpret_cast<int*>(q_over + kMaxQueries);
         const uint32_t stage = base + kOffStage + group * kStageBytes;
+        volatile int* stop = reinterpret_cast<volatile int*>(base_ptr + kOffStop) + 2 * group;        // the block and tile at which a wait ran out
         const uint32_t pitch = kTileRows * sizeof(T) + (SECTORS ? 0u : (uint32_t)ld_bytes & 15u);
         uint32_t buf = way, tph = 0;
         bool ok = true;
@@ -388,8 +424,7 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
             const int64_t b0 = (int64_t)qb * a.nb;
             const int here = a.nq - b0 < a.nb ? (int)(a.nq - b0) : a.nb;      // queries behind the last one are padding
             const int64_t mine = rt0 < row_tiles ? (row_tiles - rt0 + a.groups - 1) / a.groups : 0;
-            // the first of the block's tiles that this warp finishes: tiles are dealt to the ways in turn, across blocks
-            const int64_t first = (way - behind % ways + ways) % ways;
+            const int64_t first = first_tile(way, behind, ways);
             behind += mine;
             barrier_sync(1, 32 * kFinishWarps);
             auto keep = [&](int i, const VlQuantSide& q) {
@@ -432,9 +467,13 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
             for (int64_t rt = rt0 + first * a.groups; rt < row_tiles && ok; rt += (int64_t)ways * a.groups) {
                 const VlQuantSide held = vl_quant_side<METRIC>(next_cs, next_cn);
                 fetch(rt + (int64_t)ways * a.groups, next_cs, next_cn);
-                ok = mbar_wait(bar_tfull + 8 * buf, tph, abort_flag, a.status);
+                ok = mbar_wait(bar_tfull + 8 * buf, tph, abort_flag, a.status, a.wait_us);
                 ok = barrier_all(2 + group, 128, ok);               // the group goes on or ends as one
-                if (!ok) break;
+                if (!ok) {
+                    stop[0] = qb;
+                    stop[1] = (int)rt;
+                    break;
+                }
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * a.nb;
                 const bool fast = plain && __all_sync(0xffffffffu, held.ordinary);
@@ -481,6 +520,7 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
                 while (buf >= (uint32_t)a.accs) { buf -= a.accs; tph ^= 1u; }
             }
         }
+        if (!ok) store_none<T, SECTORS>(a, base_ptr + (stage - base), stop[0], stop[1], way, part, in_group, 2 + group);          // for the whole group
     }
     tc_fence_before();
     __syncthreads();
@@ -552,7 +592,7 @@ int launch_scan(const ScanPlan& p, const CUtensorMap& rows, const CUtensorMap& q
 }  // namespace
 
 int vl_quant_scan(const void* queries, int q_type, int64_t q_ld, const VlQuantRows& q, int64_t nq, const VlQuantRows& rows, int64_t n, int dim, int code_ld, int64_t row_lo, int64_t row_hi,
-                  void* out, int type, int64_t out_ld, int metric, int* status, cudaStream_t stream)
+                  void* out, int type, int64_t out_ld, int metric, int wait_us, int* status, cudaStream_t stream)
 {
     const EncodeTiledFn encode = vl_encode_tiled();
     VL_CHECK_ARG(encode, "vl_quant_scores: cuTensorMapEncodeTiled is not available");
@@ -602,6 +642,7 @@ int vl_quant_scan(const void* queries, int q_type, int64_t q_ld, const VlQuantRo
     a.out = out;
     a.out_ld = out_ld;
     a.status = status;
+    a.wait_us = wait_us > 0 ? wait_us : (int)(kWaitLimitNs / 1000);
     if (metric == VL_METRIC_COSINE) return launch_scan<float, VL_METRIC_COSINE>(p, map_rows, map_q, a, stream);
     if (metric == VL_METRIC_SQL2) return launch_scan<float, VL_METRIC_SQL2>(p, map_rows, map_q, a, stream);
     if (type == VL_TYPE_F32) return launch_scan<float, VL_QUANT_PRODUCT>(p, map_rows, map_q, a, stream);

@@ -36,18 +36,20 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
     return ok != 0;
 }
 // Waits for the phase of `bar` with the given parity.  False when another role raised the abort
-// flag or when the wait ran out of time (it then raises the flag itself and records the timeout).
-static __device__ __noinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status)
+// flag or when the wait ran out of time (it then raises the flag itself and records the timeout).  A try_wait
+// sleeps a while, so a limit below the usual one is looked at after each.
+static __device__ __noinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                              uint32_t limit_us = kWaitLimitNs / 1000)
 {
     unsigned long long t0 = 0;
 #pragma unroll 1
     for (uint32_t spin = 1;; ++spin) {
         if (mbar_test(bar, parity)) return true;
-        if ((spin & 63u) == 0u) {
+        if ((spin & 63u) == 0u || limit_us < kWaitLimitNs / 1000) {
             if (*abort_flag) return false;
             const unsigned long long now = now_ns();
             if (t0 == 0) t0 = now;
-            if (now - t0 > kWaitLimitNs) {
+            if (now - t0 > limit_us * 1000ull) {
                 *abort_flag = 1;
                 atomicOr(status, VL_STATUS_TIMEOUT);
                 return false;

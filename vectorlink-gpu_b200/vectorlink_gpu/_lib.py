@@ -24,7 +24,8 @@ EXPORTS = [
     "vl_queue_pop", "vl_punchout_excluded", "vl_dedup_adjacent", "vl_sort_pairs", "vl_dedup_sort_ids",
     "vl_seen_add", "vl_seen_add_noalloc", "vl_prune", "vl_prune_rows", "vl_reverse_edges", "vl_connected_components", "vl_beam_search",
     "vl_beam_search_rows", "vl_beam_search_plan", "vl_locality_keys", "vl_knn_prepare", "vl_knn_tile", "vl_knn_tile_parts",
-    "vl_quant_write", "vl_quant_read", "vl_quant_scores", "vl_quant_listed",
+    "vl_quant_write", "vl_quant_read", "vl_quant_scores", "vl_quant_scores_wait",
+    "vl_quant_listed",
 ]
 
 
@@ -90,6 +91,7 @@ def lib() -> ctypes.CDLL:
         _lib.vl_quant_write.argtypes = [P, I, L, I, L, P, L, P, P, P, L, I, P, P, P]
         _lib.vl_quant_read.argtypes = [P, P, L, I, I, P, L, L, P, I, L, P, P]
         _lib.vl_quant_scores.argtypes = [P, I, L, P, P, P, L, P, P, P, L, I, I, L, L, P, I, L, I, P, P]
+        _lib.vl_quant_scores_wait.argtypes = [P, I, L, P, P, P, L, P, P, P, L, I, I, L, L, P, I, L, I, I, P, P]
         _lib.vl_quant_listed.argtypes = [P, I, L, P, P, P, L, P, P, P, L, I, I, P, I, P, I, P, P]
         _lib.vl_beam_search.argtypes = [ctypes.POINTER(BeamParams), P]
         _lib.vl_beam_search_rows.argtypes = [ctypes.POINTER(BeamParams), P, P, P]

@@ -10,8 +10,8 @@ matters.
 
 A row that holds an infinity or a NaN is held as NaN: so is everything that is made of it.  Ids outside the store, and a
 wait inside a scan that ran out, are reported in the device's status word (`_lib.read_status`), like those of the other
-kernels.  A store belongs to the device that it was made on; its calls run on torch's current stream there.
-No gradient passes through any of this: results are data.
+kernels; results that were not made because of such a wait are NaN.  A store belongs to the device that it was made on; its
+calls run on torch's current stream there.  No gradient passes through any of this: results are data.
 """
 from __future__ import annotations
 
@@ -37,6 +37,8 @@ FEW_ROWS = 64          # rows up to which a write to places is one launch
 class QuantizedVectors:
     """`codes` int8 [count, dim to the next multiple of 16] (zeros behind `dim`), `scales` fp32 [count] and `norms` int32
     [count] (sum of squared codes).  Rows that were never written are zero."""
+
+    wait_us = 0     # longest wait inside a scan, in microseconds (0: two seconds)
 
     def __init__(self, count: int, dim: int, device="cuda"):
         self._allocate(count, dim, device, torch.zeros)
@@ -183,7 +185,8 @@ class QuantizedVectors:
         (count, q, _alive) = self._queries(queries, few if self._columns <= columns else 0)
         out = self._result(out, count, hi - lo, dtype)
         if count and hi > lo:
-            self._run("vl_quant_scores", *q, count, *self._held(), lo, hi, out.data_ptr(), TYPES[out.dtype], out.stride(0), metric)
+            self._run("vl_quant_scores_wait", *q, count, *self._held(), lo, hi, out.data_ptr(), TYPES[out.dtype], out.stride(0), metric,
+                      self.wait_us)
             if q[0] is not None and q[3] is not None:
                 _lib.LAUNCHES += 1      # the queries' codes
         return out
