@@ -111,3 +111,21 @@ def test_near_rows_are_put_in_order():
     assert same.sum() > 100
     want = (s - s[0]) ** 2 * int(store.norms[0])
     assert ((d - want).abs() <= want * 2.0 ** -24 * 1.125)[same].all()
+
+
+@pytest.mark.parametrize("dim", [1, 7, 96, 768, 1536])
+@pytest.mark.parametrize("scale", [1.0, 1e-15, 1e15])
+def test_products_are_rounded_once(dim, scale):
+    """The product of the scales has 48 digits, the whole number up to 24: all of them count.  With h = 2^-24, the part behind
+    24 digits of the scales' product is rounded by h^2 of the result, the result by h of itself."""
+    from vectorlink_gpu import QuantizedVectors
+    (q, store) = (QuantizedVectors.from_vectors(base(n, dim, n + dim, scale).to(DEV)) for n in (40, 300))
+    (qc, qs), (rc, rs) = held(q), held(store)
+    dots, got = qc @ rc.T, store.product(q).cpu().numpy()
+    assert np.array_equal(q.product(store).t().cpu().numpy(), got)
+    for i in range(40):
+        for j in range(300):
+            want = qs[i] * rs[j] * int(dots[i, j])
+            off = abs((whole([abs(got[i, j])])[0] << UNIT) - abs(want))
+            assert (got[i, j] < 0) == (want < 0) or want == 0
+            assert off << 48 <= (abs(want) << 24) + abs(want) + (1 << (UNIT + 47)), (i, j, got[i, j])

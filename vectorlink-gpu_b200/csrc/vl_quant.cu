@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(128, J > 1 ? 5 : 8) quant_listed_kernel(const 
                 }
             }
             if (m0 + lane < m_hi)
-                a.out[b * a.w + m0 + lane] = cur >= 0 ? vl_quant_pair<METRIC, true>(mine, q, vl_quant_side<METRIC>(cs, cn)) : VL_MAXFLOAT;
+                a.out[b * a.w + m0 + lane] = cur >= 0 ? vl_quant_pair<METRIC, true, false>(mine, q, vl_quant_side<METRIC>(cs, cn)) : VL_MAXFLOAT;
             cur = nxt;
         }
     }

@@ -223,7 +223,9 @@ __device__ __forceinline__ void vl_quant_rows(const T* const (&x)[R], int dim, i
 // Ordinary rows (vl_quant_ordinary) are finished in fp32.  Dots are exact there (a dot is no larger than the larger squared
 // sum, and that is at most 2^24), and the scales' product is kept as an exact pair sh + sl where 1 - t or a + b - 2 t
 // may be small against its terms:
-//   product  (qs cs) dot, two roundings
+//   product  sh f + sl f: the second product's rounding does not count, so one rounding.  Results of 16 bits (NARROW) are made of
+//            sh f alone, two roundings of 32 bits before that of 16, which is 2^13 times as large and more (500,000 x 96 x 1,000
+//            queries, bf16: 287 us, with the second product 309; 60,007 x 1536 x 4,000, fp32: 497 and 495)
 //   cosine   1/2 - sh f, rounded once by an FMA, and that - sl f: two roundings of the result itself
 //   l2       squared lengths a, b are pairs hi - over as well, hi of 20 bits, so that of rows of like length their sum is exact
 //            (otherwise its error is made exactly and summed with the rest).  2 sh f is taken from it in one FMA, and the rest
@@ -282,14 +284,14 @@ static __device__ __noinline__ float vl_quant_pair64_apart(int dot, float qs, in
 }
 // APART: what is rarely taken stands apart, and leaves the caller its registers (30,000 lists of 64 ids, 1M x 768, l2: 262 us, and
 // 274 with it inside).
-template <int METRIC, bool APART>
+template <int METRIC, bool APART, bool NARROW>
 __device__ __forceinline__ float vl_quant_pair(int dot, const VlQuantSide& q, const VlQuantSide& r)
 {
     if (q.ordinary && r.ordinary) {
         const float f = (float)dot;
-        if (METRIC == VL_QUANT_PRODUCT) return __fmul_rn(__fmul_rn(q.s, r.s), f);
-        const float cs = METRIC == VL_METRIC_COSINE ? 0.5f * r.s : 2.0f * r.s;
+        const float cs = METRIC == VL_QUANT_PRODUCT ? r.s : (METRIC == VL_METRIC_COSINE ? 0.5f * r.s : 2.0f * r.s);
         const float sh = __fmul_rn(q.s, cs), sl = __fmaf_rn(q.s, cs, -sh);
+        if (METRIC == VL_QUANT_PRODUCT) return NARROW ? __fmul_rn(sh, f) : __fmaf_rn(sh, f, __fmul_rn(sl, f));
         if (METRIC == VL_METRIC_COSINE) return __saturatef(__fmaf_rn(-sl, f, __fmaf_rn(-sh, f, 0.5f)));
         const float ab = __fadd_rn(q.hi, r.hi), of_r = __fsub_rn(ab, q.hi);
         const float more = __fadd_rn(__fsub_rn(__fsub_rn(ab, of_r), q.hi), __fsub_rn(of_r, r.hi));           // ab - a - b, exactly
@@ -309,18 +311,16 @@ __device__ __forceinline__ bool vl_quant_alike(float less, float more)
 // queries, and of the held row its scale (for cosine half of it, for l2 twice), the negative of that, and its squared length.
 // ALIKE: a + b is exact, and all are at most 16 times the shortest one.  `least` takes the smallest squared distance, or the smallest
 // excess over that of near rows where lengths vary: where it is not above that of near rows, or not above 0, vl_quant_pair has to look at them.
-template <int METRIC, bool ALIKE>
+template <int METRIC, bool NARROW, bool ALIKE>
 __device__ __forceinline__ void vl_quant_pair2(int dot0, int dot1, vl_f2 s, vl_f2 hi, vl_f2 over, vl_f2 cs, vl_f2 ncs, vl_f2 rhi, vl_f2 rover,
                                                float& r0, float& r1, float& least)
 {
     const vl_f2 f = vl_f2_pack((float)dot0, (float)dot1);
+    const vl_f2 sh = vl_f2_mul(s, cs), nsh = vl_f2_mul(s, ncs);
     if (METRIC == VL_QUANT_PRODUCT) {
-        vl_f2_unpack(vl_f2_mul(vl_f2_mul(s, cs), f), r0, r1);
-        return;
-    }
-    const vl_f2 nsh = vl_f2_mul(s, ncs);
-    if (METRIC == VL_METRIC_COSINE) {
-        const vl_f2 h = vl_f2_fma(nsh, f, vl_f2_pack(0.5f, 0.5f)), nsl = vl_f2_fma(s, ncs, vl_f2_mul(s, cs));
+        vl_f2_unpack(NARROW ? vl_f2_mul(sh, f) : vl_f2_fma(sh, f, vl_f2_mul(vl_f2_fma(s, cs, nsh), f)), r0, r1);
+    } else if (METRIC == VL_METRIC_COSINE) {
+        const vl_f2 h = vl_f2_fma(nsh, f, vl_f2_pack(0.5f, 0.5f)), nsl = vl_f2_fma(s, ncs, sh);
         float f0, f1, h0, h1, l0, l1;
         vl_f2_unpack(f, f0, f1);
         vl_f2_unpack(h, h0, h1);

@@ -230,7 +230,7 @@ static __device__ __noinline__ void hold_query(const ScanArgs& a, int b, unsigne
 }
 
 // A lane's results of a chunk: 16 queries' values are read four at a time, since shared memory feeds the products too.
-template <int METRIC, bool ALIKE>
+template <int METRIC, bool NARROW, bool ALIKE>
 __device__ __forceinline__ void finish_chunk(const uint32_t (&v)[kChunk], const float* q_scale, vl_f2 cs, vl_f2 ncs, vl_f2 hi, vl_f2 over,
                                              float (&r)[kChunk], float& least)
 {
@@ -242,17 +242,17 @@ __device__ __forceinline__ void finish_chunk(const uint32_t (&v)[kChunk], const 
             q_hi = *reinterpret_cast<const ulonglong2*>(q_scale + kMaxQueries + j);
             q_over = *reinterpret_cast<const ulonglong2*>(q_scale + 2 * kMaxQueries + j);
         }
-        vl_quant_pair2<METRIC, ALIKE>((int)v[j], (int)v[j + 1], s.x, q_hi.x, q_over.x, cs, ncs, hi, over, r[j], r[j + 1], least);
-        vl_quant_pair2<METRIC, ALIKE>((int)v[j + 2], (int)v[j + 3], s.y, q_hi.y, q_over.y, cs, ncs, hi, over, r[j + 2], r[j + 3], least);
+        vl_quant_pair2<METRIC, NARROW, ALIKE>((int)v[j], (int)v[j + 1], s.x, q_hi.x, q_over.x, cs, ncs, hi, over, r[j], r[j + 1], least);
+        vl_quant_pair2<METRIC, NARROW, ALIKE>((int)v[j + 2], (int)v[j + 3], s.y, q_hi.y, q_over.y, cs, ncs, hi, over, r[j + 2], r[j + 3], least);
     }
 }
 // ... one by one: rows that are not ordinary, and near rows among others
-template <int METRIC>
+template <int METRIC, bool NARROW>
 __device__ __forceinline__ float finish_pair(int dot, const float* q_scale, const VlQuantSide& held)
 {
     const int n = *reinterpret_cast<const int*>(q_scale + 3 * kMaxQueries);
     const VlQuantSide q = {*q_scale, q_scale[kMaxQueries], q_scale[2 * kMaxQueries], n, vl_quant_ordinary(*q_scale, n)};
-    return vl_quant_pair<METRIC, false>(dot, q, held);
+    return vl_quant_pair<METRIC, false, NARROW>(dot, q, held);
 }
 // ... and put over those in the buffer.  Not inlined: near rows are rare, and the loop over chunks has the registers for itself.
 static __device__ __noinline__ void finish_near(int4 d0, int4 d1, int4 d2, int4 d3, const float* q_scale, float row_scale, int row_n, uint32_t at, uint32_t pitch)
@@ -260,7 +260,7 @@ static __device__ __noinline__ void finish_near(int4 d0, int4 d1, int4 d2, int4 
     const VlQuantSide held = vl_quant_side<VL_METRIC_SQL2>(row_scale, row_n);
     const int dots[kChunk] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w, d2.x, d2.y, d2.z, d2.w, d3.x, d3.y, d3.z, d3.w};
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) st_shared<float>(at + j * pitch, finish_pair<VL_METRIC_SQL2>(dots[j], q_scale + j, held));
+    for (int j = 0; j < kChunk; ++j) st_shared<float>(at + j * pitch, finish_pair<VL_METRIC_SQL2, false>(dots[j], q_scale + j, held));
 }
 
 template <typename T, int METRIC, bool RESIDENT, bool SECTORS>
@@ -495,14 +495,15 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar_tempty + 8 * buf);
                     }
+                    constexpr bool kNarrow = sizeof(T) == 2;
                     float r[kChunk], least = __int_as_float(0x7f800000);
                     if (fast && alike) {
-                        finish_chunk<METRIC, true>(v, q_scale + c0, cs2, ncs2, hi2, over2, r, least);
+                        finish_chunk<METRIC, kNarrow, true>(v, q_scale + c0, cs2, ncs2, hi2, over2, r, least);
                     } else if (fast) {
-                        finish_chunk<METRIC, false>(v, q_scale + c0, cs2, ncs2, hi2, over2, r, least);
+                        finish_chunk<METRIC, kNarrow, false>(v, q_scale + c0, cs2, ncs2, hi2, over2, r, least);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < kChunk; ++j) r[j] = finish_pair<METRIC>((int)v[j], q_scale + c0 + j, held);
+                        for (int j = 0; j < kChunk; ++j) r[j] = finish_pair<METRIC, kNarrow>((int)v[j], q_scale + c0 + j, held);
                     }
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j) st_shared<T>(mine + off + j * pitch, r[j]);
