@@ -21,7 +21,7 @@ constexpr int kBlockK = 128;                   // int8 elements per k-block = on
 constexpr int kStepK = 32;                     // elements per instruction
 constexpr int kMaxStages = 12;
 constexpr int kMaxAccs = 8;                    // accumulators that tiles take in turn: 512 / nb of them
-constexpr int kChunk = 16;                     // accumulator columns (queries) that a finishing group takes at a time
+constexpr int kChunk = 16;                     // accumulator columns (queries) that a finishing group takes at a time: nb is a multiple of it
 constexpr int kParts = 4;                      // finishing groups of four warps, one per quarter of the lanes
 constexpr int kMostResident = 128;             // queries of a block that stays in shared memory: four accumulators then
 constexpr int kFinishWarps = 4 * kParts;
@@ -488,7 +488,7 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
                 for (int c0 = part * kChunk; c0 < a.nb; c0 += a.parts * kChunk, out += a.parts * kChunk * ld_bytes) {
                     const uint32_t off = SECTORS ? 0u : (uint32_t)(uintptr_t)out & 15u;
                     uint32_t v[kChunk];
-                    tc_load(taddr + c0, v);
+                    tc_load16(taddr + c0, v);
                     tc_wait_ld();
                     if (c0 + a.parts * kChunk >= a.nb) {            // the tile's last columns are in registers
                         tc_fence_before();
@@ -516,7 +516,6 @@ quant_scan_kernel(const __grid_constant__ CUtensorMap tmap_rows, const __grid_co
                     else store_rows<T, SECTORS>(out + rt * a.step * (int64_t)sizeof(T), ld_bytes, left, stage + off, pitch, in_group);
                     barrier_sync(2 + group, 128);                   // the buffer is free again
                 }
-                if (part * kChunk >= a.nb && lane == 0) mbar_arrive(bar_tempty + 8 * buf);       // nothing to finish here
                 buf += ways;
                 while (buf >= (uint32_t)a.accs) { buf -= a.accs; tph ^= 1u; }
             }
@@ -638,7 +637,7 @@ int vl_quant_scan(const void* queries, int q_type, int64_t q_ld, const VlQuantRo
     a.groups = p.groups;
     a.stages = p.stages;
     a.accs = (int)(kTmemCols / p.nb) < kMaxAccs ? (int)(kTmemCols / p.nb) : kMaxAccs;
-    a.parts = a.accs >= kParts ? 1 : 2;          // no more tiles are finished side by side than there are accumulators
+    a.parts = a.accs >= kParts ? 1 : 2;          // no more tiles are finished side by side than there are accumulators (2: more than 128 queries, enough for both parts)
     a.stage_bytes = p.stage_bytes;
     a.out = out;
     a.out_ld = out_ld;

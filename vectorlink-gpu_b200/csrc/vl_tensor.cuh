@@ -74,14 +74,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
 
-// `bytes` (a multiple of 16) from shared to global memory, both 16-byte aligned; part of the thread's open group
-__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes)
-{
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // what this thread has written to shared memory is seen by copies issued after the next barrier
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // barrier `id` of `threads` threads; true when `ok` holds in all of them
@@ -121,8 +113,6 @@ __device__ __forceinline__ void tc_load16(uint32_t taddr, uint32_t (&v)[16])
                    "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                  : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tc_load(uint32_t taddr, uint32_t (&v)[16]) { tc_load16(taddr, v); }
-__device__ __forceinline__ void tc_load(uint32_t taddr, uint32_t (&v)[32]) { tc_load32(taddr, v); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptor of a K-major tile stored as 128-byte rows (64 bf16 or 128 int8 elements) under the
