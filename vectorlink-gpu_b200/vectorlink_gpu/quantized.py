@@ -209,11 +209,11 @@ class QuantizedVectors:
         """`kernels.calculate_distances` over the held rows: out[i, j] = distance(queries[i], row beams[i, j]), MAXFLOAT
         where beams[i, j] == MAXINT."""
         (count, q, _alive) = self._queries(queries, MAXINT if self._columns <= LISTED_ROUNDS else 0)
-        # (the library takes a list's length as an int: a longer one would arrive cut to 32 bits)
-        assert beams.dim() == 2 and beams.size(1) <= MAX_LIST, f"list of up to {MAX_LIST} ids expected, got {tuple(beams.shape)}"
         beams = self._ids(beams, 2)
         (rows, width) = beams.shape
         assert rows == count
+        # (the library takes a list's length as an int: a longer one would arrive cut to 32 bits)
+        assert width <= MAX_LIST, f"list of up to {MAX_LIST} ids expected, got {width}"
         out = distances_out
         if out is None:
             out = self.codes.new_empty((rows, width), dtype=torch.float32)
