@@ -199,7 +199,7 @@ int vl_knn_tile_parts(const uint16_t* rows_bf16, int64_t n, int dim_pad, const f
  * queries [nq, dim] of q_type are held in 8 bits first, in q_codes [nq, code_ld], q_scales [nq], q_norms [nq]; with
  * queries == NULL these hold them already (up to 16 queries of up to 4096 columns need no such scratch, and up to 1536
  * columns none for vl_quant_listed: NULL).  A wait inside the kernel that runs out sets VL_STATUS_TIMEOUT in *status,
- * and what is not made by then becomes NaN.  vl_quant_scores_wait takes the longest such wait in microseconds (0: two seconds).
+ * and what is not made by then becomes NaN.  vl_quant_scores_wait takes the longest such wait in microseconds, up to two seconds (0).
  *
  * vl_quant_listed: out[b, j] = distance(queries[b], row ids[b, j]), MAXFLOAT where ids[b, j] == MAXINT (the counterpart
  * of vl_calculate_distances).  w <= 2^30. */

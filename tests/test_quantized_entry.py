@@ -66,7 +66,8 @@ def test_rows_of_a_result_that_overlap(built_lib):
         assert "overlap" in refusal("vl_quant_scores", SCORES, out_ld=out_ld)
 
 
-def test_a_negative_wait(built_lib):
+def test_waits_that_are_none_or_too_long(built_lib):
     wait = {**{k: v for k, v in SCORES.items() if k not in ("status", "stream")}, "wait_us": 0, "status": 256, "stream": None}
-    assert "wait" in refusal("vl_quant_scores_wait", wait, wait_us=-1)
+    for wait_us in (-1, 2_000_001, 2 ** 31 - 1):
+        assert "wait" in refusal("vl_quant_scores_wait", wait, wait_us=wait_us)
     assert "aligned" in refusal("vl_quant_scores_wait", wait, out=258)

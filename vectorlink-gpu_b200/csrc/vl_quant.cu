@@ -9,8 +9,11 @@ namespace {
 constexpr int kMaxDim = 131072;       // 127^2 * dim has to fit 32 bits
 
 // ---- write: one warp per row ----
-// Bound by the rows as they come: 4 bytes in and 1 out for an fp32 element (1M x 768: 560 us, 6.85 TB/s; in bf16
-// 590; 4M x 128: 914 us, 2.8 TB/s, where what has to be done per row counts).
+// Wide fp32 rows are bound by memory, 4 bytes in and 1 out for an element: 1M x 768 in 580 us, 6.7 TB/s.  The others are not: the
+// time goes by element and row, not by byte.  1M x 768 in bf16 takes 595 us, 3.9 TB/s (issue slots 74 % used, DRAM 45 %);
+// 4M x 128 913 and 923 us, 2.8 and 1.7 TB/s; 4M x 64 1,013 and 1,042.  A lane next to a half takes its warp through both ways of
+// vl_quant_codes, and the variants of several rows a warp spill 32 to 152 bytes under 64 registers.  To random places
+// 1M x 768 takes 665 and 720 us (claims and scattered rows).
 struct WriteArgs {
     const void* rows;
     int64_t m, ld;
@@ -83,8 +86,9 @@ __global__ void __launch_bounds__(256, HELD > 6 ? 2 : 4) quant_write_kernel(cons
 }
 
 // ---- read: one warp per row, four elements per lane and step ----
-// The codes of a warp's next row are on their way while the current one is stored (1M x 768 to fp32 608 us, 6.3 TB/s, to
-// bf16 371, 6.2; without them 852 and 665).
+// The codes of a warp's next row are on their way while the current one is stored (1M x 768 to fp32 610 us, 6.3 TB/s, to
+// bf16 374, 6.2; without them 852 and 665; at random ids 623 and 402).  Short rows leave lanes idle: 4M x 128 in 496 us, 5.2 TB/s, and 408,
+// 3.8 TB/s.
 template <typename T, bool VEC, int HELD>
 __global__ void __launch_bounds__(256)
 quant_read_kernel(const VlQuantRows rows, int64_t n, int dim, int code_ld, const int32_t* __restrict__ ids, int64_t first_row,
@@ -145,8 +149,9 @@ quant_read_kernel(const VlQuantRows rows, int64_t n, int dim, int code_ld, const
 // Like the gather of vl_distance.cu with rows of a quarter of the size: a row is fetched by LPR lanes, J chunks of 16 codes
 // each, several rows in flight per lane; a warp keeps its query's codes in registers, having rounded the query itself
 // (J = 0: longer rows, chunk by chunk, the query's codes from memory).  Bound by the gather of code_ld + 4 bytes per pair
-// in sectors of 32: 30,000 lists of 64 ids over 1M x 768 in 270 to 300 us, 5.0 to 5.5 TB/s; x 128 in 60 to 64 us, 4.2 to 4.5 TB/s.  A step
-// is requested when the one four (for three chunks two) ahead of it is done; five CTAs per SM for rows of two or three
+// in sectors of 32: 30,000 lists of 64 ids over 1M x 768 in 272 us (l2; cosine 311), 5.5 TB/s, with queries held before 251; x 128
+// in 73 and 64 us, 3.7 and 4.2 TB/s; 10,000 lists over 200,000 x 1536 in 159 us, 6.2 TB/s, and without rows in flight (J = 0) x 2048 in 312,
+// 4.2 TB/s, x 4096 in 628, 4.2 TB/s.  A step is requested when the one four (for three chunks two) ahead of it is done; five CTAs per SM for rows of two or three
 // chunks (four steps of three chunks, 12 warps per SM: 325 us; ids fetched step by step: 280 to 510, as the compiler orders
 // the loads).
 struct ListedArgs {
@@ -460,7 +465,7 @@ extern "C" int vl_quant_scores_wait(const void* queries, int q_type, int64_t q_l
 {
     VL_CHECK_SHAPE("vl_quant_scores", n, dim, code_ld);
     VL_CHECK_ARG(nq >= 0 && nq < VL_MAXINT, "vl_quant_scores: bad size");
-    VL_CHECK_ARG(wait_us >= 0, "vl_quant_scores: a wait of %d microseconds", wait_us);
+    VL_CHECK_ARG(wait_us >= 0 && wait_us <= 2000000, "vl_quant_scores: a wait of %d microseconds, not 0..2000000", wait_us);
     VL_CHECK_ARG(0 <= row_lo && row_lo <= row_hi && row_hi <= n, "vl_quant_scores: bad row range");
     VL_CHECK_ARG(!queries || (q_type >= VL_TYPE_F32 && q_type <= VL_TYPE_F16), "vl_quant_scores: unknown type %d", q_type);
     VL_CHECK_ARG(metric == VL_METRIC_COSINE || metric == VL_METRIC_SQL2 || metric == VL_QUANT_PRODUCT, "vl_quant_scores: unknown metric %d", metric);

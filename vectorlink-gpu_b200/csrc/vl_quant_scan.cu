@@ -5,7 +5,8 @@
 // for every query a warp stores 32 results that lie next to one another.  Which side is which also serves few
 // queries: 16 of them still fill all 128 lanes, and the scan is a stream of rows.
 //   warp 0, one lane : copies 128-column k-blocks of row tiles (and, where the queries do not fit, of the queries) into a
-//                      ring in shared memory.  The queries of a CTA's block stay in shared memory where they fit.
+//                      ring in shared memory.  A block of up to 128 queries stays in shared memory where rows have up to
+//                      three k-blocks or the block is all of them (make_plan).
 //   warp 1           : issues the products into one of the accumulators
 //   warps 2..17      : four groups that finish the scores of an accumulator each and store them
 // Waits are bounded; a wait that runs out sets VL_STATUS_TIMEOUT and ends all roles of its CTA (vl_tensor.cuh), whose results
@@ -541,11 +542,12 @@ struct ScanPlan {
 ScanPlan make_plan(int64_t nq, int kblocks, int64_t row_tiles, int sms)
 {
     ScanPlan p;
-    // A block's queries, at most 128, stay in shared memory beside four row stages if they are all of them, or if a row has few
-    // k-blocks.  Otherwise both sides stream, 256 queries at a time: shared memory feeds the products (128 x 128 x 32 reads
+    // A block's queries, at most 128, stay in shared memory beside four row stages if they are all of them, or if a row has at most
+    // three k-blocks.  Otherwise both sides stream, 256 queries at a time: shared memory feeds the products (128 x 128 x 32 reads
     // 8 KB in 64 cycles, all that it gives) and 256 columns read a quarter less for each.  100,000 rows x 2,560 queries, resident
     // and streaming: 384 elements (200,000 x 2,000) 314 and 320 us; 512 220 and 227, in bf16 210 and 171; 640 274 and 266;
-    // 768 336 and 307; 1024 (2,000 queries) 339 and 263.
+    // 768 336 and 307; 1024 (2,000 queries) 339 and 263.  The result's type is not looked at: at four k-blocks, where it
+    // matters, streaming costs 3 % in fp32 and saves 19 % in 16 bits.
     const int fit = (int)((kOperandBytes - 4 * kTileBytes) / ((uint32_t)kblocks * kBlockK)) & ~15;
     const int most = fit < kMostResident ? fit : kMostResident;
     p.resident = kblocks <= 3 || nq <= most;

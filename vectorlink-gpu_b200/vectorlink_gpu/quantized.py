@@ -38,7 +38,7 @@ class QuantizedVectors:
     """`codes` int8 [count, dim to the next multiple of 16] (zeros behind `dim`), `scales` fp32 [count] and `norms` int32
     [count] (sum of squared codes).  Rows that were never written are zero."""
 
-    wait_us = 0     # longest wait inside a scan, in microseconds (0: two seconds)
+    wait_us = 0     # longest wait inside a scan, in microseconds, up to two seconds (0)
 
     def __init__(self, count: int, dim: int, device="cuda"):
         self._allocate(count, dim, device, torch.zeros)
