@@ -11,7 +11,8 @@ matters.
 A row that holds an infinity or a NaN is held as NaN: so is everything that is made of it.  Ids outside the store, and a
 wait inside a scan that ran out, are reported in the device's status word (`_lib.read_status`), like those of the other
 kernels; results that were not made because of such a wait are NaN.  A store belongs to the device that it was made on; its
-calls run on torch's current stream there.  No gradient passes through any of this: results are data.
+calls run on torch's current stream there.  A result that the caller provides must not lie in memory that the call
+reads.  No gradient passes through any of this: results are data.
 """
 from __future__ import annotations
 
