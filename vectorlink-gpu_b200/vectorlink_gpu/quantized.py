@@ -4,9 +4,9 @@ The reference keeps fp32 rows only.  A `QuantizedVectors` holds a row as whole n
 (max|x| / 127), takes rows as they come (written as a block or to listed places), gives them back, and scores queries
 against all rows of a range or against listed ids.  Queries are held in 8 bits as well, one scale each, and the
 products of the whole numbers are summed exactly, so a pair has the same bits in `distances` and in
-`calculate_distances`, and rows that are held alike are at a squared distance of exactly 0.  The distances are those of the rows as they are held: approximations (0.4 % of the largest
-element, per element) of the fp32 rows' distances, to be scored again with `kernels.calculate_distances` where that
-matters.
+`calculate_distances`, and rows that are held alike are at a squared distance of exactly 0.  The distances are those of
+the rows as they are held: approximations (0.4 % of the largest element, per element) of the fp32 rows' distances, to be
+scored again with `kernels.calculate_distances` where that matters.
 
 A row that holds an infinity or a NaN is held as NaN: so is everything that is made of it.  Ids outside the store, and a
 wait inside a scan that ran out, are reported in the device's status word (`_lib.read_status`), like those of the other
