@@ -19,7 +19,7 @@ def scan(store, q, metric, out):
 
 # Rows of 131,072 columns: a tile takes a thousand copies, far longer than a microsecond.  40,000 queries are several blocks for a CTA.
 # The last three may or may not run out.
-@pytest.mark.parametrize("count,dim,nq,surely", [(2001, 131072, 1, True), (2001, 131072, 300, True), (1000, 131072, 20, True), (301, 8192, 40_000, True), (40_001, 96, 100, False),
+@pytest.mark.parametrize("count,dim,nq,surely", [(2001, 131072, 1, True), (2001, 131072, 300, True), (1000, 131072, 20, True), (301, 16384, 40_000, True), (40_001, 96, 100, False),
                                                  (40_001, 96, 7, False), (30_001, 1024, 600, False)])
 @pytest.mark.parametrize("metric,dtype,pad", [("l2", torch.float32, 0), ("cosine", torch.float32, 3), ("product", torch.bfloat16, 1), ("product", torch.float16, 0)])
 def test_results_that_were_not_made_are_no_numbers(count, dim, nq, surely, metric, dtype, pad):
